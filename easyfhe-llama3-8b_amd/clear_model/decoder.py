@@ -25,15 +25,37 @@ PROJECTIONS = ("q", "k", "v", "o", "gate", "up", "down")
 @dataclass
 class ClearCache:
     """Keys and values of every layer, [B, capacity, Hk, D] each, and how many of
-    a sequence's places hold one."""
+    a sequence's places hold one.
+
+    ``bound`` is the most places that the host knows a sequence to hold; None
+    where it knows nothing, as where the caller has filled the cache (whoever
+    writes ``lens`` sets it to None).  The lengths are read from the device only
+    where the bound leaves no room."""
 
     keys: list
     values: list
     lens: torch.Tensor
+    bound: int | None = None
 
     @property
     def capacity(self) -> int:
         return self.keys[0].shape[1]
+
+    def _check_batch(self, b: int) -> None:
+        if self.lens.shape != (b,):
+            raise ValueError(f"{b} sequences, a cache of {len(self.lens)}.")
+
+    def _take_place(self) -> None:
+        """Counts one more token a sequence, or refuses it.  A captured call has no
+        host to ask when it is replayed: `decode` keeps those inside the cache."""
+        if self.lens.is_cuda and torch.cuda.is_current_stream_capturing():
+            self.bound = None
+            return
+        if self.bound is None or self.bound >= self.capacity:
+            self.bound = int(self.lens.max()) if len(self.lens) else 0
+        if self.bound >= self.capacity:
+            raise ValueError(f"a sequence has no room in its cache of {self.capacity}.")
+        self.bound += 1
 
 
 def rms_norm(x, weight=None, eps: float = 1e-5):
@@ -129,21 +151,27 @@ class ClearDecoder:
     def cache(self, batch: int, capacity: int) -> ClearCache:
         new = lambda: self.embedding.new_zeros(batch, capacity, self.kv_heads, self.head_dim)  # noqa: E731
         return ClearCache([new() for _ in self.layers], [new() for _ in self.layers],
-                          torch.zeros(batch, dtype=torch.int32, device=self.embedding.device))
+                          torch.zeros(batch, dtype=torch.int32, device=self.embedding.device), 0)
 
     def logits(self, hidden):
         return _linear(rms_norm(hidden, self.final_norm, self.eps), self.lm_head)
 
     @torch.no_grad()
     def prefill(self, ids, cache: ClearCache, lens=None):
-        """Fills an empty cache with the prompts [B, T] of the given lengths, and
-        returns the logits [B, vocab] behind each prompt's last token."""
+        """Fills an empty cache with the prompts [B, T] of the given lengths (int32
+        [B]; taken as 0 below and as T beyond), and returns the logits [B, vocab]
+        behind each prompt's last token."""
+        x = self._ids(ids)
         b, t = ids.shape
+        cache._check_batch(b)
         if t > cache.capacity or t < 1:
             raise ValueError(f"prompts of {t} tokens, a cache of {cache.capacity}.")
         if lens is None:
             lens = torch.full((b,), t, dtype=torch.int32, device=ids.device)
-        x = self._ids(ids)
+        elif lens.shape != (b,) or lens.dtype != torch.int32 or lens.device != ids.device:
+            raise ValueError(f"lens is int32 [{b}] on the ids' device.")
+        else:
+            lens = lens.clamp(0, t)
         places = torch.arange(t, device=ids.device, dtype=torch.int32)
         for w, ck, cv in zip(self.layers, cache.keys, cache.values):
             q, k, v = self._qkv(w, x)
@@ -151,16 +179,21 @@ class ClearDecoder:
             ck[:, :t], cv[:, :t] = k, v
             x = self._rest(w, x, attention_forward(q, k, v, causal=True, kv_lens=lens)[0])
         cache.lens.copy_(lens)
+        cache.bound = t
         at = (lens.long() - 1).clamp(min=0)
         return self.logits(x[torch.arange(b, device=ids.device), at])
 
     @torch.no_grad()
     def decode(self, ids, cache: ClearCache):
-        """One more token [B] a sequence: its logits [B, vocab].  The caller sees to
-        it that the cache has room (its lengths stay on the device)."""
+        """One more token [B] a sequence: its logits [B, vocab].  Refused where a
+        sequence has no room left; in a replayed graph, which the host does not
+        see, a full sequence's last place is written again."""
         x = self._ids(ids[:, None])
-        rows, at = torch.arange(len(ids), device=ids.device), cache.lens.long()
-        places, lens = cache.lens[:, None], cache.lens + 1
+        cache._check_batch(len(ids))
+        cache._take_place()
+        places = cache.lens.clamp(0, cache.capacity - 1)
+        rows, at, lens = torch.arange(len(ids), device=ids.device), places.long(), places + 1
+        places = places[:, None]
         for w, ck, cv in zip(self.layers, cache.keys, cache.values):
             q, k, v = self._qkv(w, x)
             q, k = rope(self.table, q, k, positions=places)
