@@ -225,6 +225,13 @@ template <class T, int DP, int RS> struct Running {
   }
 };
 
+// log sum_j exp(s_j) of a row from its running maximum and sum (both in powers of
+// two).  The sum is 0 only where the row sees nothing, or nothing but scores of
+// -inf; NaN scores leave the maximum alone, so it is the sum that tells of them.
+__device__ __forceinline__ float row_lse(float m, float l) {
+  return l == 0.0f ? -INFINITY : (m + __log2f(l)) * LN2;
+}
+
 // Four output elements 8 b + 4 h + 0..3 of each 32, rounded once.
 template <class T, int DP>
 __device__ __forceinline__ void store_columns(T *row, const f32x16 (&o)[DP / 32], float f, int dim,
@@ -336,12 +343,11 @@ __global__ __launch_bounds__(64 * FWD_WAVES, 2) void attention_forward_kernel(At
     store_sums<DP>(p.part + (split * rows + row) * p.dim, run.o, p.dim, h);
     return;
   }
-  const float f = run.m == -INFINITY ? 0.0f : 1.0f / l;
+  const float f = l == 0.0f ? 0.0f : 1.0f / l;
   store_columns<T, DP>((T *)p.out + ((int64_t)(b * (int64_t)p.tq + qi) * p.heads + head) * p.dim,
                        run.o, f, p.dim, h);
   if (h == 0)
-    p.lse[((int64_t)b * p.heads + head) * p.tq + qi] =
-        run.m == -INFINITY ? -INFINITY : (run.m + __log2f(l)) * LN2;
+    p.lse[((int64_t)b * p.heads + head) * p.tq + qi] = row_lse(run.m, l);
 }
 
 // Few queries: the queries of a group's heads are packed into the 32 columns,
@@ -427,7 +433,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 1) void attention_few_kernel(AttnDi
 #pragma unroll
   for (int w = 0; w < FEW_WAVES; w++) {
     const float2 x = ml[w][lane & 31];
-    l += x.x == -INFINITY ? 0.0f : x.y * exp2_fast(x.x - m);
+    l += x.x == -INFINITY ? x.y : x.y * exp2_fast(x.x - m);  // x.y: 0, or NaN
   }
   const float mine = run.m == -INFINITY ? 0.0f : exp2_fast(run.m - m);
   // The waves' 32 x DP outputs: k0 and v0 are free, one wave needs DP / 32
@@ -459,7 +465,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 1) void attention_few_kernel(AttnDi
     // c is this thread's own column as lane & 31 is: m and l are that column's
     if (p.splits == 1) {
       struct alignas(8) Four { T v[4]; } y;
-      const float f = m == -INFINITY ? 0.0f : 1.0f / l;
+      const float f = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
       for (int j = 0; j < 4; j++) y.v[j] = (T)(x[j] * f);
       *(Four *)((T *)p.out + row * p.dim + quad * 4) = y;
@@ -471,8 +477,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 1) void attention_few_kernel(AttnDi
   if (tid < 32 && there) {
     const int64_t row = ((int64_t)b * p.tq + qi) * p.heads + head;
     if (p.splits == 1) {
-      p.lse[((int64_t)b * p.heads + head) * p.tq + qi] =
-          m == -INFINITY ? -INFINITY : (m + __log2f(l)) * LN2;
+      p.lse[((int64_t)b * p.heads + head) * p.tq + qi] = row_lse(m, l);
     } else {
       const int64_t rows = (int64_t)p.batch * p.tq * p.heads;
       float2 *stats = (float2 *)(p.part + p.splits * rows * p.dim);
@@ -499,10 +504,10 @@ __global__ __launch_bounds__(64) void attention_join_kernel(AttnDims p) {
   for (int x = 1; x < 64; x <<= 1) m = fmaxf(m, __shfl_xor(m, x, 64));
   for (int s = lane; s < splits; s += 64) {
     const float2 t = stats[s * rows + row];
-    l += t.x == -INFINITY ? 0.0f : t.y * exp2_fast(t.x - m);
+    l += t.x == -INFINITY ? t.y : t.y * exp2_fast(t.x - m);  // t.y: 0, or NaN
   }
   for (int x = 1; x < 64; x <<= 1) l += __shfl_xor(l, x, 64);
-  const float inv = m == -INFINITY ? 0.0f : 1.0f / l;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   for (int d = 2 * lane; d < p.dim; d += 128) {
     float a0 = 0.0f, a1 = 0.0f;
 #pragma unroll 4
@@ -516,8 +521,7 @@ __global__ __launch_bounds__(64) void attention_join_kernel(AttnDims p) {
     y[0] = (T)(a0 * inv), y[1] = (T)(a1 * inv);
   }
   if (lane == 0)
-    p.lse[((int64_t)b * p.heads + head) * p.tq + qi] =
-        m == -INFINITY ? -INFINITY : (m + __log2f(l)) * LN2;
+    p.lse[((int64_t)b * p.heads + head) * p.tq + qi] = row_lse(m, l);
 }
 
 // ----------------------------------------------------------------- backward

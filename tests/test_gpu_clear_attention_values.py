@@ -1,0 +1,60 @@
+"""Grouped attention of the clear decoder on values at the types' borders: NaN and
+infinities that a query sees."""
+
+from __future__ import annotations
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import clear_plain as plain  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+BF16, FP16 = torch.bfloat16, torch.float16
+
+
+def _inputs(b, n, m, h, kv, d, t, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return [torch.randn(b, x, y, d, generator=g, device="cuda").to(t)
+            for x, y in ((n, h), (m, kv), (m, kv), (n, h))]
+
+
+# one block and several for packed queries, then for whole tiles of them; the
+# keys [a, b) are all that one wave, or one block, takes
+SEEN = [(1, 100, 4, 2, 32, 64), (1, 3000, 4, 2, 256, 512), (200, 300, 4, 2, 64, 128),
+        (1100, 1600, 1, 1, 320, 640), (3, 64, 4, 2, 0, 64), (200, 64, 4, 2, 0, 64)]
+
+
+@pytest.mark.parametrize("t", [BF16, FP16])
+@pytest.mark.parametrize("n,m,h,kv,a,b", SEEN)
+def test_nan_that_a_query_sees_is_in_its_lse(n, m, h, kv, a, b, t):
+    """-inf is for queries that see nothing."""
+    import clear_model as cm
+
+    q, k, v, _ = _inputs(2, n, m, h, kv, 64, t, 1)
+    val, err = plain.attention(q, k, v, False)
+    k[1, a:b] = float("nan")
+    q[0, n // 2, h - 1] = float("nan")
+    out, lse = cm.attention_forward(q, k, v, causal=False)
+    assert bool(torch.isnan(lse[1]).all()) and bool(torch.isnan(out[1]).all())
+    assert bool(torch.isnan(lse[0, h - 1, n // 2])) and bool(torch.isnan(out[0, n // 2, h - 1]).all())
+    keep = torch.ones(n, h, dtype=torch.bool, device="cuda")
+    keep[n // 2, h - 1] = False
+    plain.assert_within(out[0][keep], val[0][0][keep], err[0][0][keep], "out")
+    plain.assert_within(lse[0].t()[keep], val[1][0].t()[keep], err[1][0].t()[keep], "lse")
+
+
+@pytest.mark.parametrize("t", [BF16, FP16])
+@pytest.mark.parametrize("n,m,h,kv,a,b", SEEN[:4])
+def test_a_score_of_minus_infinity_takes_its_key_out(n, m, h, kv, a, b, t):
+    import clear_model as cm
+
+    q, k, v, _ = _inputs(1, n, m, h, kv, 64, t, 2)
+    q[..., 0] = 1.0
+    keep = torch.ones(m, dtype=torch.bool, device="cuda")
+    keep[a:b], keep[-1] = False, False
+    val, err = plain.attention(q, k[:, keep], v[:, keep], False)
+    k[:, ~keep, :, 0] = float("-inf")
+    out, lse = cm.attention_forward(q, k, v, causal=False)
+    plain.assert_within(out, val[0], err[0], "out")
+    plain.assert_within(lse, val[1], err[1], "lse")
