@@ -124,10 +124,20 @@ __device__ __forceinline__ void row_operand(typename Half<T>::x8 (&f)[DP / 16], 
 
 // ------------------------------------------------------------------ forward
 
+// A probability enters the second product rounded to the inputs' type, as 2^UP
+// times its power relative to a maximum that lags by up to 2^SLACK.  fp16 has no
+// numbers below 2^-25: carried up to its largest ones, powers down to 2^-38 of a
+// row's largest count, so that 2^20 small ones are not lost behind one key with
+// most of the mass.  (Relative to the maximum alone, as bf16 takes them, 40000
+// keys of 2^-26 round to an output of 0 in place of 6e-4.)
+template <class T> struct Powers;
+template <> struct Powers<__bf16> { static constexpr float SLACK = 8.0f, UP = 0.0f; };
+template <> struct Powers<_Float16> { static constexpr float SLACK = 2.0f, UP = 13.0f; };
+
 // Running softmax of one query column over 32 RS keys, and the output's update.
 template <class T, int DP, int RS> struct Running {
   f32x16 o[DP / 32];
-  float m, l;
+  float m, l;  // o and l carry 2^UP until `finish`, which puts it into m
 
   __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -136,6 +146,7 @@ template <class T, int DP, int RS> struct Running {
       for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
     m = -INFINITY, l = 0.0f;
   }
+  __device__ __forceinline__ void finish() { l = halves_sum(l), m -= Powers<T>::UP; }
 
   // The K and V tiles' first row is key0, and the column sees keys below
   // `limit` (`masked`, the same for the wave) or all of them.
@@ -177,9 +188,9 @@ template <class T, int DP, int RS> struct Running {
 #pragma unroll
       for (int i = 0; i < 16; i++) top = fmaxf(top, s[r][i]);
     top = halves_max(top) * scale2;
-    // The maximum only has to keep the powers in range: it moves when the new
-    // one is more than 2^8 above, so most steps leave the outputs as they are.
-    if (__any(top > m + 8.0f)) {
+    // The maximum only has to keep the powers in range: it moves when the new one
+    // is more than the slack above, so most steps leave the outputs as they are.
+    if (__any(top > m + Powers<T>::SLACK)) {
       const float next = fmaxf(m, top);
       const float f = m == -INFINITY ? 0.0f : exp2_fast(m - next);
       l *= f;
@@ -189,7 +200,7 @@ template <class T, int DP, int RS> struct Running {
         for (int i = 0; i < 16; i++) o[d][i] *= f;
       m = next;
     }
-    const float shift = m == -INFINITY ? 0.0f : m;
+    const float shift = m == -INFINITY ? 0.0f : m - Powers<T>::UP;
     auto powers = [&](int r) {
       float sum = 0.0f;
 #pragma unroll
@@ -334,7 +345,8 @@ __global__ __launch_bounds__(64 * FWD_WAVES, 2) void attention_forward_kernel(At
     if (key + FWD_KEYS < end) use(key + FWD_KEYS, k1, v1);
   }
   if (!there) return;
-  const float l = halves_sum(run.l);
+  run.finish();
+  const float l = run.l;
   if (p.splits > 1) {
     const int64_t rows = (int64_t)p.batch * p.tq * p.heads;
     const int64_t row = ((int64_t)b * p.tq + qi) * p.heads + head;
@@ -424,7 +436,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 1) void attention_few_kernel(AttnDi
     use(key, kw0, vw0);
   }
   // Join: every wave's outputs relative to the common maximum.
-  run.l = halves_sum(run.l);
+  run.finish();
   if (h == 0) ml[wave][lane & 31] = make_float2(run.m, run.l);
   __syncthreads();
   float m = -INFINITY, l = 0.0f;

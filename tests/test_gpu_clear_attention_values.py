@@ -1,7 +1,9 @@
 """Grouped attention of the clear decoder on values at the types' borders: NaN and
-infinities that a query sees."""
+infinities that a query sees, and long tails of small probabilities."""
 
 from __future__ import annotations
+
+import math
 
 import pytest
 
@@ -58,3 +60,30 @@ def test_a_score_of_minus_infinity_takes_its_key_out(n, m, h, kv, a, b, t):
     out, lse = cm.attention_forward(q, k, v, causal=False)
     plain.assert_within(out, val[0], err[0], "out")
     plain.assert_within(lse, val[1], err[1], "lse")
+
+
+@pytest.mark.parametrize("t", [BF16, FP16])
+@pytest.mark.parametrize("n,h,m,first", [(1, 4, 200000, True), (1, 4, 200000, False),
+                                         (200, 1, 40000, True), (200, 1, 40000, False),
+                                         (4096, 8, 40000, True), (4096, 8, 40000, False)])
+def test_a_long_tail_of_small_probabilities(n, h, m, first, t):
+    """One key with nearly all of the mass in front of or behind many with 2^-26 of
+    it each: the values of the many are all that the output holds.
+
+    Each probability is rounded once to the type, which keeps 2^-26 of a row's
+    largest within half a step u; sums are fp32."""
+    import clear_model as cm
+
+    d = 64
+    q = torch.ones(1, n, h, d, dtype=t, device="cuda")
+    k, v = torch.zeros(1, m, 1, d, dtype=t, device="cuda"), torch.ones(1, m, 1, d, dtype=t, device="cuda")
+    at = 0 if first else m - 1
+    k[:, at], v[:, at] = 2.25, 0.0  # a score of 18
+    out, lse = cm.attention_forward(q, k, v, causal=False)
+    tail = (m - 1) * math.exp(-18.0)
+    want, u = tail / (1.0 + tail), plain.half_step(t)
+    # a probability's rounding and the result's; the power's argument, and a sum
+    # of m equal numbers in fp32
+    bound = want * (2 * u + (64 + m) * plain.F32)
+    assert float((out.double() - want).abs().max()) <= bound
+    assert float((lse.double() - math.log(1.0 + tail) - 18.0).abs().max()) <= (80 + m) * plain.F32
