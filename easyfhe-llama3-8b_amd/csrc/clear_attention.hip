@@ -546,8 +546,48 @@ constexpr int BWD_WAVES = 4;
 // it in fp16, where do . v decides its size.
 constexpr float P_LOG = 15.0f, P_UP = 32768.0f;
 template <class T> struct Carried;
-template <> struct Carried<__bf16> { static constexpr float DOWN = 1.0f, LEFT = 1.0f / P_UP; };
-template <> struct Carried<_Float16> { static constexpr float DOWN = 1.0f / P_UP, LEFT = 1.0f; };
+template <> struct Carried<__bf16> {
+  static constexpr float DOWN = 1.0f, LEFT = 1.0f / P_UP;
+  static constexpr bool ENDS = false;
+};
+template <> struct Carried<_Float16> {
+  static constexpr float DOWN = 1.0f / P_UP, LEFT = 1.0f;
+  static constexpr bool ENDS = true;
+};
+
+// Arrays that a lambda holds by reference stay in registers only if it is inlined.
+#define INLINE __attribute__((always_inline))
+
+// In fp16 a score gradient may be beyond the largest number where the sums that
+// it goes into, times the scale, are not: a column's sums are then infinite or
+// NaN in every element (infinity times 0 is NaN), so one of them tells.  The
+// block takes such columns again, in units of 2^13 and at last of 2^26, which
+// hold any do . v of fp16 operands (128 x 2^32, twice).  What that loses, below
+// 2^-12 of a number beyond 2^16 (2 of one beyond 2^29), is less than the large
+// one's rounding.  Calls without such a column pay a vote of each block: 1 us a
+// kernel where blocks are short, 2 x 4096 causal tokens with 32 and 8 heads of
+// 128 forward and backward 1.28 -> 1.30 ms.
+constexpr float FEWER = 1.0f / 8192.0f, FEWEST = FEWER * FEWER;
+__device__ __forceinline__ bool column_lost(float x) { return !(halves_sum(x * 0.0f) == 0.0f); }
+
+// pass(), and again with smaller units as long as columns are lost.  `votes` has a
+// place for each of the block's waves; a pass that is taken again has barriers.
+template <class T, int WAVES, class P, class X>
+__device__ __forceinline__ void passes(float &unit, int *votes, P &&pass, X &&sum) {
+  for (;;) {
+    pass();
+    if constexpr (!Carried<T>::ENDS) break;
+    const bool lost = column_lost(sum()) && unit > FEWEST;
+    votes[threadIdx.x >> 6] = __any(lost);
+    __syncthreads();
+    int any = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) any |= votes[w];
+    // the same for all lanes: matrix products have no place in a divergent loop
+    if (__builtin_expect(!uniform(any), 1)) break;
+    unit *= lost ? FEWER : 1.0f;
+  }
+}
 
 // dq of 128 queries of one head, and each query's (lse, delta) for the keys'
 // gradients.  The columns are queries, so both statistics are the lane's own.
@@ -570,6 +610,7 @@ __global__ __launch_bounds__(64 * BWD_WAVES, 2) void attention_dq_kernel(AttnDim
   constexpr int ROWS = 32 * BWD_WAVES, KEYS = 64;
   __shared__ __attribute__((aligned(16))) T k0[KEYS * L::PITCH], k1[KEYS * L::PITCH];
   __shared__ __attribute__((aligned(16))) T v0[KEYS * L::PITCH], v1[KEYS * L::PITCH];
+  __shared__ int votes[BWD_WAVES];
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), h = lane >> 5, c = lane & 31;
   const int pairs = p.batch * p.kv_heads;
   const int pair = blockIdx.x % pairs, part = blockIdx.x / pairs % p.dq_parts;
@@ -614,10 +655,8 @@ __global__ __launch_bounds__(64 * BWD_WAVES, 2) void attention_dq_kernel(AttnDim
   const T *kb = (const T *)p.k + b * p.k_sb + kvh * p.k_sh;
   const T *vb = (const T *)p.v + b * p.v_sb + kvh * p.v_sh;
   f32x16 dq[DP / 32];
-#pragma unroll
-  for (int d = 0; d < DP / 32; d++)
-#pragma unroll
-    for (int i = 0; i < 16; i++) dq[d][i] = 0.0f;
+  float unit = 1.0f;  // that the column's score gradients are in
+  bool again = false;
   Rows<T, DP, KEYS, 64 * BWD_WAVES> krows, vrows;
   krows.open(kb, p.k_st, p.dim, tid), vrows.open(vb, p.v_st, p.dim, tid);
   auto load = [&](int key, T *k, T *v) {
@@ -657,7 +696,8 @@ __global__ __launch_bounds__(64 * BWD_WAVES, 2) void attention_dq_kernel(AttnDim
     const int64_t n = (int64_t)p.batch * p.heads * p.tq;
     p.stat[at] = lse2, p.stat[n + at] = delta;
   }
-  auto use = [&](int key, const T *k, const T *v) {
+  float down = Carried<T>::DOWN, shift = 0.0f;
+  auto use = [&](int key, const T *k, const T *v) INLINE {
     if (key >= closed) return;
     rd.renew();
     f32x16 s[2], dp[2];
@@ -673,8 +713,7 @@ __global__ __launch_bounds__(64 * BWD_WAVES, 2) void attention_dq_kernel(AttnDim
     auto gradients = [&](int r) {
 #pragma unroll
       for (int i = 0; i < 16; i++)
-        s[r][i] = exp2_fast(fmaf(s[r][i], p.scale2, -lse2)) *
-                  fmaf(dp[r][i], Carried<T>::DOWN, -delta);
+        s[r][i] = exp2_fast(fmaf(s[r][i], p.scale2, -lse2)) * fmaf(dp[r][i], down, -shift);
     };
     auto add = [&](int r) {
 #pragma unroll
@@ -712,15 +751,31 @@ __global__ __launch_bounds__(64 * BWD_WAVES, 2) void attention_dq_kernel(AttnDim
     interleave<DP / 16, 4, 2>();
     __builtin_amdgcn_sched_barrier(0);
   };
-  for (int key = begin; key < end; key += 2 * KEYS) {
-    tile_barrier();
-    if (key + KEYS < end && !few) load(key + KEYS, k1, v1);
-    use(key, k0, v0);
-    tile_barrier();
-    if (key + 2 * KEYS < end) load(key + 2 * KEYS, k0, v0);
-    if (key + KEYS < end) use(key + KEYS, k1, v1);
-  }
+  auto pass = [&]() INLINE {
+    down = Carried<T>::DOWN * unit, shift = delta * unit;
+#pragma unroll
+    for (int d = 0; d < DP / 32; d++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) dq[d][i] = 0.0f;
+    if (again && begin < end && !few) load(begin, k0, v0);
+    for (int key = begin; key < end; key += 2 * KEYS) {
+      tile_barrier();
+      if (key + KEYS < end && !few) load(key + KEYS, k1, v1);
+      use(key, k0, v0);
+      tile_barrier();
+      if (key + 2 * KEYS < end) load(key + 2 * KEYS, k0, v0);
+      if (key + KEYS < end) use(key + KEYS, k1, v1);
+    }
+    again = true;
+  };
+  passes<T, BWD_WAVES>(unit, votes, pass, [&] { return dq[0][0]; });
   if (there && p.dq_parts > 1) {
+    if constexpr (Carried<T>::ENDS) {
+#pragma unroll
+      for (int d = 0; d < DP / 32; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) dq[d][i] *= 1.0f / unit;
+    }
     const int64_t rows = (int64_t)p.batch * p.tq * p.heads;
     store_sums<DP>(p.dq_part + (part * rows + ((int64_t)b * p.tq + qi) * p.heads + head) * p.dim, dq,
                    p.dim, h);
@@ -728,7 +783,7 @@ __global__ __launch_bounds__(64 * BWD_WAVES, 2) void attention_dq_kernel(AttnDim
   }
   if (there)
     store_columns<T, DP>((T *)p.dq + ((int64_t)(b * (int64_t)p.tq + qi) * p.heads + head) * p.dim,
-                         dq, p.scale * Carried<T>::LEFT, p.dim, h);
+                         dq, p.scale * Carried<T>::LEFT / unit, p.dim, h);
 }
 
 // dk and dv of 32 WAVES keys of one key head: the columns are keys, and the group's
@@ -756,6 +811,7 @@ __global__ __launch_bounds__(128 * WAVES, 2) void attention_dkv_kernel(AttnDims 
   __shared__ __attribute__((aligned(16))) T d0[ROWS * L::PITCH], d1[ROWS * L::PITCH];
   __shared__ __attribute__((aligned(16))) T vt[COLS * L::PITCH];
   __shared__ __attribute__((aligned(16))) float st0[2 * 64], st1[2 * 64];
+  __shared__ int votes[2 * WAVES];
   const int tid = threadIdx.x, set = uniform(tid / (64 * WAVES)), lane = tid & 63, wave = uniform(tid >> 6) & (WAVES - 1), h = lane >> 5, c = lane & 31;
   const int pairs = p.batch * p.kv_heads;
   const int pair = blockIdx.x % pairs;
@@ -769,10 +825,8 @@ __global__ __launch_bounds__(128 * WAVES, 2) void attention_dkv_kernel(AttnDims 
   row_operand<T, DP>(kf, (const T *)p.k + b * p.k_sb + (int64_t)key * p.k_st + kvh * p.k_sh, there,
                      p.dim, h);
   f32x16 dk[DP / 32], dv[DP / 32];
-#pragma unroll
-  for (int d = 0; d < DP / 32; d++)
-#pragma unroll
-    for (int i = 0; i < 16; i++) dk[d][i] = 0.0f, dv[d][i] = 0.0f;
+  float unit = 1.0f;  // that the column's score gradients are in
+  bool again = false;
   // queries that see a key of this block, and the first that sees any key
   const int lo = p.causal ? max(0, -off) : 0;
   const int from = p.causal ? max(lo, first_key - off) : 0;
@@ -786,8 +840,9 @@ __global__ __launch_bounds__(128 * WAVES, 2) void attention_dkv_kernel(AttnDims 
   qrows.open((const T *)p.q + b * p.q_sb, p.q_st, p.dim, tid);
   drows.open((const T *)p.dout + b * p.o_sb, p.o_st, p.dim, tid);
   // the next step's head of the group and first row
-  int load_head = steps > 0 ? first_step / per_head : 0;
-  int load_row = from + (first_step - load_head * per_head) * ROWS, use_row = load_row;
+  const int head0 = steps > 0 ? first_step / per_head : 0;
+  const int row0 = from + (first_step - head0 * per_head) * ROWS;
+  int load_head, load_row, use_row;
   auto load = [&](T *qt, T *dt, float *st) {
     const int head = kvh * p.group + load_head;
     qrows.load(head * p.q_sh, load_row, p.tq, qt, tid);
@@ -804,7 +859,7 @@ __global__ __launch_bounds__(128 * WAVES, 2) void attention_dkv_kernel(AttnDims 
   };
   Reads<T, DP> rd;
   rd.open(lane);
-  auto use = [&](const T *qt, const T *dt, const float *st) {
+  auto use = [&](const T *qt, const T *dt, const float *st) INLINE {
     rd.renew();
     const int row0 = use_row;
     use_row = use_row + ROWS >= p.tq ? from : use_row + ROWS;
@@ -837,6 +892,10 @@ __global__ __launch_bounds__(128 * WAVES, 2) void attention_dkv_kernel(AttnDims 
           s[i] = e;
         }
       }
+      if (Carried<T>::ENDS && again) {
+#pragma unroll
+        for (int i = 0; i < 16; i++) dp[i] *= unit;
+      }
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int kk = 0; kk < 2; kk++) {
@@ -859,15 +918,31 @@ __global__ __launch_bounds__(128 * WAVES, 2) void attention_dkv_kernel(AttnDims 
     Rows<T, DP, COLS, THREADS> vrows;
     vrows.open((const T *)p.v + b * p.v_sb + kvh * p.v_sh, p.v_st, p.dim, tid);
     vrows.load(0, first_key, len, vt, tid);
-    load(q0, d0, st0);
   }
-  for (int i = 0; i < steps; i += 2) {
-    tile_barrier();
-    if (i + 1 < steps) load(q1, d1, st1);
-    use(q0, d0, st0);
-    tile_barrier();
-    if (i + 2 < steps) load(q0, d0, st0);
-    if (i + 1 < steps) use(q1, d1, st1);
+  auto pass = [&]() INLINE {
+#pragma unroll
+    for (int d = 0; d < DP / 32; d++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) dk[d][i] = 0.0f, dv[d][i] = 0.0f;
+    load_head = head0, load_row = use_row = row0;
+    if (steps > 0) load(q0, d0, st0);
+    for (int i = 0; i < steps; i += 2) {
+      tile_barrier();
+      if (i + 1 < steps) load(q1, d1, st1);
+      use(q0, d0, st0);
+      tile_barrier();
+      if (i + 2 < steps) load(q0, d0, st0);
+      if (i + 1 < steps) use(q1, d1, st1);
+    }
+    again = true;
+  };
+  // columns from the sequence's length on hold what nobody reads
+  passes<T, 2 * WAVES>(unit, votes, pass, [&] { return there ? dk[0][0] : 0.0f; });
+  if constexpr (Carried<T>::ENDS) {
+#pragma unroll
+    for (int d = 0; d < DP / 32; d++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) dk[d][i] *= 1.0f / unit;
   }
   // dk, then dv, from the second set to the first through the row buffers'
   // space; q0 .. d1 are one set's 4 waves x 32 keys x DP floats at DP = PITCH.

@@ -1,5 +1,6 @@
 """Grouped attention of the clear decoder on values at the types' borders: NaN and
-infinities that a query sees, and long tails of small probabilities."""
+infinities that a query sees, long tails of small probabilities, and score
+gradients beyond fp16's largest number."""
 
 from __future__ import annotations
 
@@ -87,3 +88,50 @@ def test_a_long_tail_of_small_probabilities(n, h, m, first, t):
     bound = want * (2 * u + (64 + m) * plain.F32)
     assert float((out.double() - want).abs().max()) <= bound
     assert float((lse.double() - math.log(1.0 + tail) - 18.0).abs().max()) <= (80 + m) * plain.F32
+
+
+@pytest.mark.parametrize("b,n,m,h,kv,d,causal", [
+    (1, 90, 100, 4, 2, 64, False), (1, 70, 128, 4, 2, 128, False), (1, 90, 300, 4, 2, 64, True),
+    (2, 300, 633, 4, 2, 80, True), (1, 1031, 2400, 4, 1, 128, True), (1, 203, 403, 4, 4, 40, False),
+])
+def test_score_gradients_beyond_fp16(b, n, m, h, kv, d, causal):
+    """Scores' gradients above 65504 whose sums, times the scale, are within it: in
+    some rows and keys, beside others of every smaller size."""
+    import clear_model as cm
+
+    q, k, v, do = _inputs(b, n, m, h, kv, d, FP16, 3)
+    scale = 0.004
+    v = (v.float() * (4e4 * m / (1000.0 * math.sqrt(d)))).to(FP16)
+    do = (do.float() * torch.logspace(-1, 3, n, device="cuda")[None, :, None, None]).to(FP16)
+    val, err = plain.attention(q, k, v, causal, scale=scale, dout=do)
+    # the largest score gradient of the first sequence's first head
+    s = (q[0, :, 0].double() @ k[0, :, 0].double().t()) * scale
+    s = s.masked_fill(~plain.visible(1, n, m, causal, None, None, "cuda")[0], float("-inf"))
+    ds = torch.softmax(s, 1) * (do[0, :, 0].double() @ v[0, :, 0].double().t()
+                                - (do[0, :, 0].double() * val[0][0, :, 0]).sum(1, keepdim=True))
+    assert float(ds.abs().max()) > 65504.0
+    assert all(float(x.abs().max()) < 65504.0 for x in val[2:])
+    out, lse = cm.attention_forward(q, k, v, causal=causal, scale=scale)
+    grads = cm.attention_backward(do, q, k, v, out, lse, causal=causal, scale=scale)
+    for name, got, y, e in zip(("out", "lse", "dq", "dk", "dv"), (out, lse) + grads, val, err):
+        plain.assert_within(got, y, e, name)
+
+
+@pytest.mark.parametrize("n,m,h,kv,d", [(30, 40, 4, 2, 64), (130, 200, 2, 2, 128)])
+def test_the_largest_score_gradients_of_fp16(n, m, h, kv, d):
+    """Operands at the end of fp16, and a scale that brings the results back."""
+    import clear_model as cm
+
+    q, k, v, do = _inputs(1, n, m, h, kv, d, FP16, 4)
+    v, do = (torch.sign(x) * 6e4 for x in (v, do))
+    do = do * torch.logspace(-4, 0, n, device="cuda")[None, :, None, None]
+    v, do, scale = v.to(FP16), do.to(FP16), 1e-6
+    val, err = plain.attention(q, k, v, False, scale=scale, dout=do)
+    # v - out at the flat probabilities, of the last and largest row
+    far = do[0, -1, 0].double() @ (v[0, :, 0].double() - val[0][0, -1, 0]).t() / m
+    assert float(far.abs().max()) > 65504.0 * 2 ** 13
+    assert all(float(x.abs().max()) < 65504.0 for x in val[2:])
+    out, lse = cm.attention_forward(q, k, v, causal=False, scale=scale)
+    grads = cm.attention_backward(do, q, k, v, out, lse, causal=False, scale=scale)
+    for name, got, y, e in zip(("dq", "dk", "dv"), grads, val[2:], err[2:]):
+        plain.assert_within(got, y, e, name)
