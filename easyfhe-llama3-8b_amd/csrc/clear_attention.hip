@@ -651,7 +651,9 @@ __global__ __launch_bounds__(64 * BWD_WAVES, 2) void attention_dq_kernel(AttnDim
     }
   }
   const int64_t at = ((int64_t)b * p.heads + head) * p.tq + qi;
-  const float lse2 = live ? fmaf(p.lse[at], LOG2E, -P_LOG) : INFINITY;
+  // nor does one that sees nothing but scores of -inf, whose output is 0 as well
+  const float lse = live ? p.lse[at] : -INFINITY;
+  const float lse2 = lse == -INFINITY ? INFINITY : fmaf(lse, LOG2E, -P_LOG);
   const T *kb = (const T *)p.k + b * p.k_sb + kvh * p.k_sh;
   const T *vb = (const T *)p.v + b * p.v_sb + kvh * p.v_sh;
   f32x16 dq[DP / 32];

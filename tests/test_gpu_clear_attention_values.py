@@ -63,6 +63,26 @@ def test_a_score_of_minus_infinity_takes_its_key_out(n, m, h, kv, a, b, t):
     plain.assert_within(lse, val[1], err[1], "lse")
 
 
+@pytest.mark.parametrize("n,m", [(5, 100), (200, 300), (200, 100)])
+def test_nothing_but_scores_of_minus_infinity(n, m):
+    """Finite operands whose products leave fp32: an output of 0, lse = -inf, and no
+    part in any gradient."""
+    import clear_model as cm
+
+    q, k, v, do = _inputs(1, n, m, 2, 1, 64, BF16, 5)
+    q.zero_(), k.fill_(1e20)
+    q[0, 2, 1] = -1e20
+    out, lse = cm.attention_forward(q, k, v, causal=False)
+    dq, dk, dv = cm.attention_backward(do, q, k, v, out, lse, causal=False)
+    assert float(out[0, 2, 1].abs().max()) == 0.0 and float(lse[0, 1, 2]) == float("-inf")
+    assert float(dq[0, 2, 1].abs().max()) == 0.0 and bool(torch.isfinite(dq).all())
+    assert float(dk.abs().max()) == 0.0  # the others' queries are 0
+    rest = do.clone()
+    rest[0, 2, 1] = 0.0
+    val, err = plain.attention(torch.zeros_like(q), k, v, False, dout=rest)
+    plain.assert_within(dv, val[4], err[4], "dv")
+
+
 @pytest.mark.parametrize("t", [BF16, FP16])
 @pytest.mark.parametrize("n,h,m,first", [(1, 4, 200000, True), (1, 4, 200000, False),
                                          (200, 1, 40000, True), (200, 1, 40000, False),
