@@ -141,9 +141,9 @@ class ClearDecoder:
 
     def score(self, hidden, targets, *, ignore_index: int = -100):
         """Losses [N] of final hidden states [N, hidden], such as a decrypted
-        prefill's, before the final norm."""
-        x = rms_norm(torch.as_tensor(hidden).to(self.lm_head.device, self.lm_head.dtype),
-                     self.final_norm, self.eps)
+        prefill's, before the final norm: normed in fp32, then rounded once."""
+        x = rms_norm(torch.as_tensor(hidden).to(self.lm_head.device, torch.float32),
+                     self.final_norm, self.eps).to(self.lm_head.dtype)
         return linear_cross_entropy_forward(x, self.lm_head, targets, ignore_index=ignore_index)[0]
 
     # ------------------------------------------------------------ generating

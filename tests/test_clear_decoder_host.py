@@ -103,3 +103,30 @@ def test_prefill_refusals(model):
         model.decode(_ids(1, 1)[:, 0], model.cache(2, 8))
     with pytest.raises(ValueError, match="ids"):
         model.prefill(_ids(2, 3)[0], model.cache(2, 8))
+
+
+@pytest.mark.parametrize("t", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("norm", [False, True])
+def test_scored_states_are_rounded_once(model, monkeypatch, t, norm):
+    """Decrypted states come in fp64, some far beyond fp16: what the loss gets is
+    the normed state in 64 bits, off by half a step of the type and fp32's share."""
+    got = []
+    monkeypatch.setattr(dec, "linear_cross_entropy_forward",
+                        lambda x, *a, **kw: got.append(x) or (None, None))
+    model.lm_head = model.lm_head.to(t)
+    g = torch.Generator().manual_seed(1)
+    h = torch.randn(50, D, generator=g, dtype=torch.float64)
+    h[:, 3] *= 3e5
+    w = torch.rand(D, generator=g) + 0.5 if norm else None
+    model.final_norm = w
+    model.score(h, torch.zeros(50, dtype=torch.int64))
+    model.score(h.numpy(), torch.zeros(50, dtype=torch.int64))
+    want = h * torch.rsqrt(h.square().mean(-1, keepdim=True) + 1e-5)
+    if norm:
+        want = want * w.double()
+    u, tiny = torch.finfo(t).eps / 2, torch.finfo(t).smallest_normal * torch.finfo(t).eps / 2
+    # the state to fp32, the mean of D squares and its root, two products
+    bound = want.abs() * (u + (D / 2 + 8) * 2.0 ** -24) + tiny
+    for x in got:
+        assert x.dtype is t and bool(((x.double() - want).abs() <= bound).all())
+    assert len(got) == 2
