@@ -81,6 +81,17 @@ def check(rc: int) -> None:
     raise OperatorError(msg)
 
 
+_grad_enabled = torch.is_grad_enabled
+
+
+def without_graph(name: str, x, y=None, z=None) -> None:
+    """The plain entry points leave no graph: refused where one would be missed.
+    (Written out: a generator over the tensors would cost a small call 1 us.)"""
+    if _grad_enabled() and (x.requires_grad or y is not None and y.requires_grad
+                            or z is not None and z.requires_grad):
+        raise ValueError(f"a tensor requires gradients: use {name} for them, or torch.no_grad().")
+
+
 # torch's own compiled code asks for the current stream's handle this way; the
 # public route through a Stream object costs 2 us, a tenth of a small call.
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (

@@ -90,7 +90,9 @@ def attention_forward(q, k, v, *, causal: bool, kv_lens=None, q_start=None, scal
     without it; what a cache holds beyond is not read into the result) and,
     where ``causal``, j <= i + q_start[b] (int32; Tk - Tq without it, which
     puts the last query at the last key).  A query that sees nothing gets
-    zeros and lse = -inf.  ``scale`` is 1/sqrt(D) unless given."""
+    zeros and lse = -inf.  ``scale`` is 1/sqrt(D) unless given.  No graph is
+    kept: tensors that require gradients go through ``attention``."""
+    _native.without_graph("attention", q, k, v)
     lens, starts, scale, _held = _checked(q, k, v, kv_lens, q_start, scale)
     q, qs = _rows(q)
     k, ks = _rows(k)

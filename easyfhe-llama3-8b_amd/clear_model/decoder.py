@@ -139,6 +139,7 @@ class ClearDecoder:
         return linear_cross_entropy(x.reshape(-1, x.shape[-1]), self.lm_head, targets.reshape(-1),
                                     ignore_index=ignore_index, reduction=reduction)
 
+    @torch.no_grad()
     def score(self, hidden, targets, *, ignore_index: int = -100):
         """Losses [N] of final hidden states [N, hidden], such as a decrypted
         prefill's, before the final norm: normed in fp32, then rounded once."""

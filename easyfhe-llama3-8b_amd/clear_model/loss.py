@@ -67,7 +67,9 @@ def _run(fn, backward, hidden, weight, targets, ptrs, ignore_index):
 def linear_cross_entropy_forward(hidden, weight, targets, *, ignore_index: int = -100):
     """(loss, lse), fp32 [N], of hidden [N, D] through weight [V, D] at the int64
     targets [N].  Where the target is ``ignore_index`` both are 0; where it is
-    no class the loss is NaN."""
+    no class the loss is NaN.  No graph is kept: tensors that require gradients
+    go through ``linear_cross_entropy``."""
+    _native.without_graph("linear_cross_entropy", hidden, weight)
     _checked(hidden, weight, targets)
     n = hidden.shape[0]
     loss = hidden.new_empty(n, dtype=torch.float32)

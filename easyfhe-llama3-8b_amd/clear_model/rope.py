@@ -132,7 +132,9 @@ def _rope(table: RopeTable, q, k, positions, inverse: bool):
 def rope(table: RopeTable, q, k=None, *, positions):
     """(q', k') of q [B, T, H, D] and k [B, T, Hk, D] (or None) at the integer
     positions [T] or [B, T].  Any strides; the results are new and contiguous.
-    Angles are reduced in fp64, the result is rounded once."""
+    Angles are reduced in fp64, the result is rounded once.  No graph is kept:
+    tensors that require gradients go through ``apply_rope``."""
+    _native.without_graph("apply_rope", q, k)
     return _rope(table, q, k, positions, False)
 
 
