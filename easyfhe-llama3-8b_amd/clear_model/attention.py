@@ -57,8 +57,8 @@ def _checked(q, k, v, kv_lens, q_start, scale):
         q_start = _per_sequence("q_start", q_start, b, dev)
         starts = q_start.data_ptr()
     scale = d ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < 1e30:
-        raise ValueError("the scale is positive and finite.")
+    if not 1.1754943508222875e-38 <= scale < 1e30:
+        raise ValueError("the scale is positive and finite in fp32.")
     # the tensors are returned too: they live until the call has been made
     return lens, starts, scale, (kv_lens, q_start)
 

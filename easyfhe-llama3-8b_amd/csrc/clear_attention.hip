@@ -1021,7 +1021,9 @@ static AttnDims attention_dims(const clear_attention_args &a) {
           "attention: the query heads are a multiple of the key heads");
   require(a.dim >= 8 && a.dim <= 128 && a.dim % 8 == 0,
           "attention: the head is a multiple of 8, at most 128");
-  require(a.scale > 0 && a.scale < 1e30, "attention: the scale is positive and finite");
+  // FLT_MIN: below it the scale has fewer bits in fp32, or is 0
+  require(a.scale >= 1.1754943508222875e-38 && a.scale < 1e30,
+          "attention: the scale is positive and finite in fp32");
   const int64_t most = (int64_t)1 << 30;
   require(a.batch <= most && a.q_tokens <= most && a.kv_tokens <= most && a.heads <= 1 << 16 &&
               a.batch * a.heads <= most, "attention: too large");

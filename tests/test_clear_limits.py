@@ -1,0 +1,29 @@
+"""Borders of what the clear decoder's attention takes, on the host alone."""
+
+from __future__ import annotations
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from clear_model import _native  # noqa: E402
+from clear_model.attention import _checked  # noqa: E402
+from test_clear_model import _attention_args, _Fake  # noqa: E402
+
+
+@pytest.mark.parametrize("scale", [1e-46, 1e-39])
+def test_scales_below_fp32(scale):
+    """In fp32 such a scale is 0 or loses its bits, and a hidden key's -inf times 0
+    is NaN."""
+    with pytest.raises(ValueError, match="scale"):
+        _native.check(_native.lib.clear_attention_forward(_attention_args(scale=scale), None))
+    x = _Fake(torch.zeros(1, 2, 4, 64, dtype=torch.bfloat16))
+    with pytest.raises(ValueError, match="scale"):
+        _checked(x, x, x, None, None, scale)
+
+
+def test_the_smallest_scale():
+    n = _native.query(_native.lib.clear_attention_workspace, _attention_args(scale=1.2e-38), False)
+    assert n == 0
+    x = _Fake(torch.zeros(1, 2, 4, 64, dtype=torch.bfloat16))
+    assert _checked(x, x, x, None, None, 1.2e-38)[2] == 1.2e-38
