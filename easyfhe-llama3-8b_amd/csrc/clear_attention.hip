@@ -37,7 +37,8 @@ struct AttnDims {
 __device__ __forceinline__ int visible_len(const AttnDims &p, int b) {
   return p.kv_lens ? min(max(p.kv_lens[b], 0), p.tk) : p.tk;
 }
-// Query i sees keys up to i + offset (kept where i + offset cannot overflow).
+// Query i sees keys up to i + offset (kept where i + offset cannot overflow: the
+// host sees to it that queries and keys together leave a tile below 2^31).
 __device__ __forceinline__ int causal_offset(const AttnDims &p, int b) {
   return p.q_start ? min(max(p.q_start[b], -p.tq), p.tk) : p.tk - p.tq;
 }
@@ -1026,7 +1027,8 @@ static AttnDims attention_dims(const clear_attention_args &a) {
           "attention: the scale is positive and finite in fp32");
   const int64_t most = (int64_t)1 << 30;
   require(a.batch <= most && a.q_tokens <= most && a.kv_tokens <= most && a.heads <= 1 << 16 &&
-              a.batch * a.heads <= most, "attention: too large");
+              a.batch * a.heads <= most && a.q_tokens + a.kv_tokens <= 2 * most - 256,
+          "attention: too large");
   AttnDims p = {};
   p.q = a.q, p.k = a.k, p.v = a.v, p.out = a.out, p.lse = (float *)a.lse;
   p.kv_lens = (const int *)a.kv_lens, p.q_start = (const int *)a.q_start;

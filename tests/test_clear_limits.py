@@ -27,3 +27,16 @@ def test_the_smallest_scale():
     assert n == 0
     x = _Fake(torch.zeros(1, 2, 4, 64, dtype=torch.bfloat16))
     assert _checked(x, x, x, None, None, 1.2e-38)[2] == 1.2e-38
+
+
+@pytest.mark.parametrize("n,m,fits", [(1 << 30, 1 << 30, False), (1 << 30, (1 << 30) - 256, True)])
+def test_places_of_queries_have_31_bits(n, m, fits):
+    """A query's last visible key, its place plus the start (at most the keys), is
+    computed in 32 bits, up to a whole tile beyond the last query."""
+    args = _attention_args(n=n, m=m, h=1, kv=1, d=8, causal=1)
+    if fits:
+        assert _native.query(_native.lib.clear_attention_workspace, args, True) > 0
+        return
+    for backward in (False, True):
+        with pytest.raises(ValueError, match="large"):
+            _native.query(_native.lib.clear_attention_workspace, args, backward)
