@@ -32,3 +32,12 @@ BF16, FP16 = torch.bfloat16, torch.float16
 def test_every_kind_of_tile(n, v, d, ignored, t):
     x, w, y, dl = _inputs(n, v, d, t, ignored, seed=30, scale=1024.0 if t == FP16 else 1.0)
     _check(x, w, y, dl)
+
+
+@pytest.mark.parametrize("t", [BF16, FP16])
+@pytest.mark.parametrize("n,v,d,ignored", [(1 << 14, 300, 64, 0.4), (40001, 300, 64, 0.4),
+                                           (70000, 129, 72, 0.9), (131072, 130, 8, 0.0)])
+def test_lists_of_many_tokens(n, v, d, ignored, t):
+    """Blocks of 16, 39, 68 and 128 tokens, taken 64 at a time."""
+    x, w, y, dl = _inputs(n, v, d, t, ignored, seed=31, scale=1024.0 if t == FP16 else 1.0)
+    _check(x, w, y, dl)
