@@ -556,37 +556,48 @@ template <> struct Carried<_Float16> {
   static constexpr bool ENDS = true;
 };
 
-// Arrays that a lambda holds by reference stay in registers only if it is inlined.
-#define INLINE __attribute__((always_inline))
-
 // In fp16 a score gradient may be beyond the largest number where the sums that
 // it goes into, times the scale, are not: a column's sums are then infinite or
 // NaN in every element (infinity times 0 is NaN), so one of them tells.  The
 // block takes such columns again, in units of 2^13 and at last of 2^26, which
 // hold any do . v of fp16 operands (128 x 2^32, twice).  What that loses, below
 // 2^-12 of a number beyond 2^16 (2 of one beyond 2^29), is less than the large
-// one's rounding.  Calls without such a column pay a vote of each block: 1 us a
-// kernel where blocks are short, 2 x 4096 causal tokens with 32 and 8 heads of
-// 128 forward and backward 1.28 -> 1.30 ms.
+// one's rounding.
 constexpr float FEWER = 1.0f / 8192.0f, FEWEST = FEWER * FEWER;
-__device__ __forceinline__ bool column_lost(float x) { return !(halves_sum(x * 0.0f) == 0.0f); }
 
-// pass(), and again with smaller units as long as columns are lost.  `votes` has a
-// place for each of the block's waves; a pass that is taken again has barriers.
-template <class T, int WAVES, class P, class X>
-__device__ __forceinline__ void passes(float &unit, int *votes, P &&pass, X &&sum) {
-  for (;;) {
-    pass();
-    if constexpr (!Carried<T>::ENDS) break;
-    const bool lost = column_lost(sum()) && unit > FEWEST;
-    votes[threadIdx.x >> 6] = __any(lost);
-    __syncthreads();
-    int any = 0;
+// Whether a column of the block is lost, the same for all of its lanes; those lanes
+// whose own is get the next unit.
+template <int WAVES> __device__ __forceinline__ bool lost_columns(float sum, float &unit, int *votes) {
+  const bool lost = !(halves_sum(sum * 0.0f) == 0.0f) && unit > FEWEST;
+  votes[threadIdx.x >> 6] = __any(lost);
+  __syncthreads();
+  int any = 0;
 #pragma unroll
-    for (int w = 0; w < WAVES; w++) any |= votes[w];
-    // the same for all lanes: matrix products have no place in a divergent loop
-    if (__builtin_expect(!uniform(any), 1)) break;
-    unit *= lost ? FEWER : 1.0f;
+  for (int w = 0; w < WAVES; w++) any |= votes[w];
+  unit *= lost ? FEWER : 1.0f;
+  return uniform(any) != 0;
+}
+
+// block(dims, thread, block, unit, again) until it returns false.  Nearly every
+// call takes nothing again and should not pay for it with registers: its arguments
+// and its place are hidden from the compiler, which would keep what follows from
+// them for the next time.  5 x 1003 uneven tokens with 12 heads of 64, forward and
+// backward, of four sets of lengths: 52-83 us without any of this, 53-84 with it,
+// 53-94 where nothing is hidden (a block less a CU); 2 x 4096 causal tokens of 32
+// and 8 heads of 128 1.304, 1.310 and 1.34 ms; 4 x 128 of them 44, 46 and 47 us.
+template <class T, class F> __device__ __forceinline__ void blocks(const AttnDims &p, F &&block) {
+  float unit = 1.0f;
+  if constexpr (!Carried<T>::ENDS) {
+    block(p, (int)threadIdx.x, (int)blockIdx.x, unit, false);
+  } else {
+    for (bool again = false;; again = true) {
+      // the kernel's one argument
+      typedef const __attribute__((address_space(4))) AttnDims *Argument;
+      Argument a = (Argument)__builtin_amdgcn_kernarg_segment_ptr();
+      int thread = threadIdx.x, index = blockIdx.x;
+      asm volatile("" : "+s"(a), "+v"(thread), "+s"(index));
+      if (__builtin_expect(!block(*(const AttnDims *)a, thread, index, unit, again), 1)) break;
+    }
   }
 }
 
@@ -606,16 +617,15 @@ __device__ __forceinline__ void passes(float &unit, int *votes, P &&pass, X &&su
 // PFLOP/s, the matrix units busy 60% of the cycles at 1.75 GHz (one half at a
 // time: 421 us).
 template <class T, int DP>
-__global__ __launch_bounds__(64 * BWD_WAVES, 2) void attention_dq_kernel(AttnDims p) {
+__device__ __forceinline__ bool dq_block(const AttnDims &p, int tid, int block, float &unit) {
   using L = Tile<DP>;
   constexpr int ROWS = 32 * BWD_WAVES, KEYS = 64;
   __shared__ __attribute__((aligned(16))) T k0[KEYS * L::PITCH], k1[KEYS * L::PITCH];
   __shared__ __attribute__((aligned(16))) T v0[KEYS * L::PITCH], v1[KEYS * L::PITCH];
-  __shared__ int votes[BWD_WAVES];
-  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), h = lane >> 5, c = lane & 31;
+  const int lane = tid & 63, wave = uniform(tid >> 6), h = lane >> 5, c = lane & 31;
   const int pairs = p.batch * p.kv_heads;
-  const int pair = blockIdx.x % pairs, part = blockIdx.x / pairs % p.dq_parts;
-  const int rest = blockIdx.x / pairs / p.dq_parts;
+  const int pair = block % pairs, part = block / pairs % p.dq_parts;
+  const int rest = block / pairs / p.dq_parts;
   const int b = pair / p.kv_heads, kvh = pair % p.kv_heads;
   const int tiles = (p.tq + ROWS - 1) / ROWS;
   const int q0 = (tiles - 1 - rest / p.group) * ROWS;
@@ -658,8 +668,10 @@ __global__ __launch_bounds__(64 * BWD_WAVES, 2) void attention_dq_kernel(AttnDim
   const T *kb = (const T *)p.k + b * p.k_sb + kvh * p.k_sh;
   const T *vb = (const T *)p.v + b * p.v_sb + kvh * p.v_sh;
   f32x16 dq[DP / 32];
-  float unit = 1.0f;  // that the column's score gradients are in
-  bool again = false;
+#pragma unroll
+  for (int d = 0; d < DP / 32; d++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) dq[d][i] = 0.0f;
   Rows<T, DP, KEYS, 64 * BWD_WAVES> krows, vrows;
   krows.open(kb, p.k_st, p.dim, tid), vrows.open(vb, p.v_st, p.dim, tid);
   auto load = [&](int key, T *k, T *v) {
@@ -699,8 +711,9 @@ __global__ __launch_bounds__(64 * BWD_WAVES, 2) void attention_dq_kernel(AttnDim
     const int64_t n = (int64_t)p.batch * p.heads * p.tq;
     p.stat[at] = lse2, p.stat[n + at] = delta;
   }
-  float down = Carried<T>::DOWN, shift = 0.0f;
-  auto use = [&](int key, const T *k, const T *v) INLINE {
+  // the score gradients' unit, which is 1 unless they are taken again
+  const float down = Carried<T>::DOWN * unit, shift = delta * unit;
+  auto use = [&](int key, const T *k, const T *v) {
     if (key >= closed) return;
     rd.renew();
     f32x16 s[2], dp[2];
@@ -754,39 +767,42 @@ __global__ __launch_bounds__(64 * BWD_WAVES, 2) void attention_dq_kernel(AttnDim
     interleave<DP / 16, 4, 2>();
     __builtin_amdgcn_sched_barrier(0);
   };
-  auto pass = [&]() INLINE {
-    down = Carried<T>::DOWN * unit, shift = delta * unit;
-#pragma unroll
-    for (int d = 0; d < DP / 32; d++)
-#pragma unroll
-      for (int i = 0; i < 16; i++) dq[d][i] = 0.0f;
-    if (again && begin < end && !few) load(begin, k0, v0);
-    for (int key = begin; key < end; key += 2 * KEYS) {
-      tile_barrier();
-      if (key + KEYS < end && !few) load(key + KEYS, k1, v1);
-      use(key, k0, v0);
-      tile_barrier();
-      if (key + 2 * KEYS < end) load(key + 2 * KEYS, k0, v0);
-      if (key + KEYS < end) use(key + KEYS, k1, v1);
-    }
-    again = true;
-  };
-  passes<T, BWD_WAVES>(unit, votes, pass, [&] { return dq[0][0]; });
-  if (there && p.dq_parts > 1) {
-    if constexpr (Carried<T>::ENDS) {
+  for (int key = begin; key < end; key += 2 * KEYS) {
+    tile_barrier();
+    if (key + KEYS < end && !few) load(key + KEYS, k1, v1);
+    use(key, k0, v0);
+    tile_barrier();
+    if (key + 2 * KEYS < end) load(key + 2 * KEYS, k0, v0);
+    if (key + KEYS < end) use(key + KEYS, k1, v1);
+  }
+  if constexpr (Carried<T>::ENDS) {
+    __shared__ int votes[BWD_WAVES];
+    const float used = unit;
+    if (lost_columns<BWD_WAVES>(dq[0][0], unit, votes)) return true;
+    if (p.dq_parts > 1) {
 #pragma unroll
       for (int d = 0; d < DP / 32; d++)
 #pragma unroll
-        for (int i = 0; i < 16; i++) dq[d][i] *= 1.0f / unit;
+        for (int i = 0; i < 16; i++) dq[d][i] *= 1.0f / used;
     }
+  }
+  if (there && p.dq_parts > 1) {
     const int64_t rows = (int64_t)p.batch * p.tq * p.heads;
     store_sums<DP>(p.dq_part + (part * rows + ((int64_t)b * p.tq + qi) * p.heads + head) * p.dim, dq,
                    p.dim, h);
-    return;
+    return false;
   }
   if (there)
     store_columns<T, DP>((T *)p.dq + ((int64_t)(b * (int64_t)p.tq + qi) * p.heads + head) * p.dim,
                          dq, p.scale * Carried<T>::LEFT / unit, p.dim, h);
+  return false;
+}
+
+template <class T, int DP>
+__global__ __launch_bounds__(64 * BWD_WAVES, 2) void attention_dq_kernel(AttnDims p) {
+  blocks<T>(p, [](const AttnDims &a, int tid, int block, float &unit, bool) {
+    return dq_block<T, DP>(a, tid, block, unit);
+  });
 }
 
 // dk and dv of 32 WAVES keys of one key head: the columns are keys, and the group's
@@ -807,20 +823,19 @@ __global__ __launch_bounds__(64 * BWD_WAVES, 2) void attention_dq_kernel(AttnDim
 // a block: the queries are then shared out over `parts` blocks a tile, whose
 // fp32 sums a second kernel adds in order.
 template <class T, int DP, int WAVES>
-__global__ __launch_bounds__(128 * WAVES, 2) void attention_dkv_kernel(AttnDims p) {
+__device__ __forceinline__ bool dkv_block(const AttnDims &p, int tid, int block, float &unit, bool again) {
   using L = Tile<DP>;
   constexpr int COLS = 32 * WAVES, ROWS = 64, THREADS = 128 * WAVES;
   __shared__ __attribute__((aligned(16))) T q0[ROWS * L::PITCH], q1[ROWS * L::PITCH];
   __shared__ __attribute__((aligned(16))) T d0[ROWS * L::PITCH], d1[ROWS * L::PITCH];
   __shared__ __attribute__((aligned(16))) T vt[COLS * L::PITCH];
   __shared__ __attribute__((aligned(16))) float st0[2 * 64], st1[2 * 64];
-  __shared__ int votes[2 * WAVES];
-  const int tid = threadIdx.x, set = uniform(tid / (64 * WAVES)), lane = tid & 63, wave = uniform(tid >> 6) & (WAVES - 1), h = lane >> 5, c = lane & 31;
+  const int set = uniform(tid / (64 * WAVES)), lane = tid & 63, wave = uniform(tid >> 6) & (WAVES - 1), h = lane >> 5, c = lane & 31;
   const int pairs = p.batch * p.kv_heads;
-  const int pair = blockIdx.x % pairs;
+  const int pair = block % pairs;
   const int b = pair / p.kv_heads, kvh = pair % p.kv_heads;
-  const int part = blockIdx.x / pairs % p.parts;
-  const int first_key = blockIdx.x / pairs / p.parts * COLS;  // the longest first
+  const int part = block / pairs % p.parts;
+  const int first_key = block / pairs / p.parts * COLS;  // the longest first
   const int key = first_key + wave * 32 + c;
   const int len = visible_len(p, b), off = causal_offset(p, b);
   const bool there = key < len;
@@ -828,8 +843,10 @@ __global__ __launch_bounds__(128 * WAVES, 2) void attention_dkv_kernel(AttnDims 
   row_operand<T, DP>(kf, (const T *)p.k + b * p.k_sb + (int64_t)key * p.k_st + kvh * p.k_sh, there,
                      p.dim, h);
   f32x16 dk[DP / 32], dv[DP / 32];
-  float unit = 1.0f;  // that the column's score gradients are in
-  bool again = false;
+#pragma unroll
+  for (int d = 0; d < DP / 32; d++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) dk[d][i] = 0.0f, dv[d][i] = 0.0f;
   // queries that see a key of this block, and the first that sees any key
   const int lo = p.causal ? max(0, -off) : 0;
   const int from = p.causal ? max(lo, first_key - off) : 0;
@@ -843,9 +860,8 @@ __global__ __launch_bounds__(128 * WAVES, 2) void attention_dkv_kernel(AttnDims 
   qrows.open((const T *)p.q + b * p.q_sb, p.q_st, p.dim, tid);
   drows.open((const T *)p.dout + b * p.o_sb, p.o_st, p.dim, tid);
   // the next step's head of the group and first row
-  const int head0 = steps > 0 ? first_step / per_head : 0;
-  const int row0 = from + (first_step - head0 * per_head) * ROWS;
-  int load_head, load_row, use_row;
+  int load_head = steps > 0 ? first_step / per_head : 0;
+  int load_row = from + (first_step - load_head * per_head) * ROWS, use_row = load_row;
   auto load = [&](T *qt, T *dt, float *st) {
     const int head = kvh * p.group + load_head;
     qrows.load(head * p.q_sh, load_row, p.tq, qt, tid);
@@ -862,7 +878,7 @@ __global__ __launch_bounds__(128 * WAVES, 2) void attention_dkv_kernel(AttnDims 
   };
   Reads<T, DP> rd;
   rd.open(lane);
-  auto use = [&](const T *qt, const T *dt, const float *st) INLINE {
+  auto use = [&](const T *qt, const T *dt, const float *st) {
     rd.renew();
     const int row0 = use_row;
     use_row = use_row + ROWS >= p.tq ? from : use_row + ROWS;
@@ -921,31 +937,27 @@ __global__ __launch_bounds__(128 * WAVES, 2) void attention_dkv_kernel(AttnDims 
     Rows<T, DP, COLS, THREADS> vrows;
     vrows.open((const T *)p.v + b * p.v_sb + kvh * p.v_sh, p.v_st, p.dim, tid);
     vrows.load(0, first_key, len, vt, tid);
+    load(q0, d0, st0);
   }
-  auto pass = [&]() INLINE {
-#pragma unroll
-    for (int d = 0; d < DP / 32; d++)
-#pragma unroll
-      for (int i = 0; i < 16; i++) dk[d][i] = 0.0f, dv[d][i] = 0.0f;
-    load_head = head0, load_row = use_row = row0;
-    if (steps > 0) load(q0, d0, st0);
-    for (int i = 0; i < steps; i += 2) {
-      tile_barrier();
-      if (i + 1 < steps) load(q1, d1, st1);
-      use(q0, d0, st0);
-      tile_barrier();
-      if (i + 2 < steps) load(q0, d0, st0);
-      if (i + 1 < steps) use(q1, d1, st1);
-    }
-    again = true;
-  };
-  // columns from the sequence's length on hold what nobody reads
-  passes<T, 2 * WAVES>(unit, votes, pass, [&] { return there ? dk[0][0] : 0.0f; });
+  for (int i = 0; i < steps; i += 2) {
+    tile_barrier();
+    if (i + 1 < steps) load(q1, d1, st1);
+    use(q0, d0, st0);
+    tile_barrier();
+    if (i + 2 < steps) load(q0, d0, st0);
+    if (i + 1 < steps) use(q1, d1, st1);
+  }
   if constexpr (Carried<T>::ENDS) {
+    __shared__ int votes[2 * WAVES];
+    const float used = unit;
+    // columns from the sequence's length on hold what nobody reads
+    if (lost_columns<2 * WAVES>(there ? dk[0][0] : 0.0f, unit, votes)) return true;
+    if (again) {
 #pragma unroll
-    for (int d = 0; d < DP / 32; d++)
+      for (int d = 0; d < DP / 32; d++)
 #pragma unroll
-      for (int i = 0; i < 16; i++) dk[d][i] *= 1.0f / unit;
+        for (int i = 0; i < 16; i++) dk[d][i] *= 1.0f / used;
+    }
   }
   // dk, then dv, from the second set to the first through the row buffers'
   // space; q0 .. d1 are one set's 4 waves x 32 keys x DP floats at DP = PITCH.
@@ -978,7 +990,7 @@ __global__ __launch_bounds__(128 * WAVES, 2) void attention_dkv_kernel(AttnDims 
         }
     }
   }
-  if (set == 1 || key >= p.tk) return;
+  if (set == 1 || key >= p.tk) return false;
   const int64_t row = ((int64_t)b * p.tk + key) * p.kv_heads + kvh;
   if (!there) {  // keys beyond the sequence's length have had no part
 #pragma unroll
@@ -990,10 +1002,18 @@ __global__ __launch_bounds__(128 * WAVES, 2) void attention_dkv_kernel(AttnDims 
     const int64_t rows = (int64_t)p.batch * p.tk * p.kv_heads;
     float *out = p.part + (2 * part * rows + row) * p.dim;
     store_sums<DP>(out, dk, p.dim, h), store_sums<DP>(out + rows * p.dim, dv, p.dim, h);
-    return;
+    return false;
   }
   store_columns<T, DP>((T *)p.dk + row * p.dim, dk, p.scale * Carried<T>::LEFT, p.dim, h);
   store_columns<T, DP>((T *)p.dv + row * p.dim, dv, 1.0f / P_UP, p.dim, h);
+  return false;
+}
+
+template <class T, int DP, int WAVES>
+__global__ __launch_bounds__(128 * WAVES, 2) void attention_dkv_kernel(AttnDims p) {
+  blocks<T>(p, [](const AttnDims &a, int tid, int block, float &unit, bool again) {
+    return dkv_block<T, DP, WAVES>(a, tid, block, unit, again);
+  });
 }
 
 // The sum of the parts' [parts][stride] values, in order, times f, rounded once.
