@@ -2,10 +2,13 @@
 the encrypted programs evaluate, in bf16 and fp16, with their gradients.
 
 What the encrypted prefill computes on ciphertexts runs here on plain tensors:
-for calibration, for checking a decrypted result, for generating after an
-encrypted prompt, and for adapting weights before they are encoded.  The
-operators are hand-written gfx950 kernels (``libclear_mi355x.so``) on torch
-tensors; ``ClearDecoder`` runs them together.
+for scoring decrypted hidden states, for generating after an encrypted prompt,
+and for adapting weights before they are encoded.  (16 bits are too coarse to
+check a decrypted result with; that is done in fp64, and so is calibration,
+which needs every layer's intermediates.)  Rotary positions, attention and the
+vocabulary loss are hand-written gfx950 kernels (``libclear_mi355x.so``) on
+torch tensors; ``ClearDecoder`` runs them together, with torch's products and
+norms between them.
 """
 
 from .attention import attention, attention_backward, attention_forward

@@ -1,9 +1,10 @@
 """ctypes binding of libclear_mi355x.so (include/clear_mi355x.h).
 
-The library is the only compute path: if it is missing this module raises at
-import, so nothing can silently fall back to torch's own operators.  The
-operators take torch tensors, and torch is imported first: the library binds
-to the HIP runtime that torch has loaded.
+The library is the only compute path of rotary positions, attention and the
+vocabulary loss: if it is missing this module raises at import, and none of
+them falls back to torch's own operators.  (``ClearDecoder`` does its norms,
+projections and SiLU with torch.)  The operators take torch tensors, and torch
+is imported first: the library binds to the HIP runtime that torch has loaded.
 """
 
 from __future__ import annotations

@@ -12,8 +12,8 @@
 // two more products take g to dx (summed in fp32 over the pieces) and dw.  The
 // largest entry of a row of g is nearly always the target's, so its rounding is
 // nearly all of g's: what it took off is kept in fp32 and added to both
-// gradients at the end (error of the gradients' 2-norm in bf16 2.5e-3 without,
-// 1.8e-3 with it, of which 1.7e-3 is the result's own rounding).
+// gradients at the end (error of the gradients' 2-norm in bf16 2.5e-3 without and
+// 1.7e-3 with it, as of rounding the result alone).
 // Rows with the ignored target are left out of every product: the first kernel
 // lists the others, and the products run over that list.
 #include "clear_device.hpp"
@@ -812,7 +812,9 @@ static LossPlan plan_loss(const clear_loss_args &a, bool backward, LossDims &p, 
   // copies and products shorten: 5 x 15061 x 4000 63 us whole, 57 in halves; 300 x
   // 2000 x 3000 46 and 31; as many as the CUs (128 x 32000 x 4096): 79 and 77.
   plan.classes = p.direct && !backward && small_tiles < 256 ? 64 : plan.tile;
-  // A piece's g stays within 256 MB; all pieces have about the same size.
+  // A piece's g takes up to 256 MB, and from 32768 tokens on 8 KB a token: fewer
+  // than 4096 classes would have dx's sums read and written for too few products.
+  // All pieces have about the same size.
   const int64_t most_piece = std::max<int64_t>(4096, ((int64_t)1 << 27) / n / 256 * 256);
   const int64_t pieces = ceil_div(a.vocab, most_piece);
   plan.piece = (int)(ceil_div(ceil_div(a.vocab, pieces), 256) * 256);
